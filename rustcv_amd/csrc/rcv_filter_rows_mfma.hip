@@ -706,8 +706,7 @@ struct FRItem {                // (all scalar)
 // Round 6, same-process A/B on four boxes (profiles/r06_chain_variants.txt): CV_PACK2 -0.9 ... -1.2 % on three, +0.2 % on one -- with it the
 // filter runs level with its own memory-only form.  Built, measured and removed again: twelve more VALU instructions per step +0.2 % (an
 // instruction costs next to nothing here); a second, discarded ticket draw per item from a line of the same XCD and queue +0.1 % (a draw costs
-// nothing measurable); the next item's ticket requested three steps ahead and waited for at the item's end 0 ... +0.4 % (and the pending
-// scalar register pair is invisible to the compiler: not worth the hazard).
+// nothing measurable).
 constexpr int CV_PACK2 = 1, CV_TRACE = 32;
 constexpr int kChainVar = CV_PACK2;   // the product's form
 template <int KS, int PP, bool EDGE, int DBG, int DMASK, int VAR>
@@ -731,15 +730,27 @@ __device__ __forceinline__ void fr_chain_run(const FRArgs& a, const int lane, co
     unsigned long long* const tick = a.tickets + 16 * (2 * xcd + (EDGE ? 1 : 0));
     const unsigned long long inv_k = EDGE ? a.inv_edge : a.inv_int;
 
-    // A ticket is drawn with a SCALAR atomic (s_atomic_add_x2, returns the old value): its latency is counted by lgkmcnt, which
-    // nothing else in the loop uses, so waiting for it on the spot stalls this wave's issue for one L2 round trip per item (the other
-    // wave of the SIMD runs on) but leaves vmcnt alone -- the row pairs in flight stay in flight.  (A vector atomic drawn one item
-    // ahead was built first: the compiler's atomic optimizer broadcasts the result at the draw site behind an s_waitcnt vmcnt(0),
-    // which drains the prefetch ring once per item.)
-    auto draw = [&]() -> unsigned {
-        unsigned long long t = 1ull;
-        asm volatile("s_atomic_add_x2 %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(t) : "s"(tick) : "memory");
-        return (unsigned)t;   // items per launch < 2^31 (host check)
+    // A ticket is a returning VECTOR atomic of one lane (this library only ever reads through the scalar data cache), requested ahead of its
+    // use: `ask` sends it at the head of a trip of the loop below, `take` reads it kLead steps later.  vmcnt is in order, and by then
+    // `prepare` has waited for a row pair requested AFTER the ticket, so the compiler needs no wait there, or one that leaves the younger row
+    // pairs in flight (vmcnt(9) and up).  An item is at least a trip long (host: item_rows), so a trip enters at most one item and one ticket
+    // at a time is enough.  The address goes through a VGPR the compiler cannot see through: for a uniform one its atomic optimizer
+    // broadcasts the result at the draw behind an s_waitcnt vmcnt(0), which drains the prefetch ring once per item.
+    constexpr int kLead = PP + 1;
+    static_assert(kLead < RP, "the ticket is read in the trip that asked for it");
+    unsigned tick_off = 0;
+    asm volatile("" : "+v"(tick_off));
+    unsigned long long tv = 0;               // (lane 0) the ticket asked for
+    unsigned ticket = 0;                     // the ticket read
+    int state = 0;                           // 0: none, 1: asked for, 2: read
+    auto ask = [&]() {
+        if (lane == 0) tv = __hip_atomic_fetch_add((unsigned long long*)((uint8_t*)tick + tick_off), 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        state = 1;
+        asm volatile("" : "+s"(state));      // (keeps the join of the lane branch apart from the caller's: merged, the state counts as divergent)
+    };
+    auto take = [&]() {
+        ticket = (unsigned)__builtin_amdgcn_readfirstlane((int)tv);   // items per launch < 2^31 (host check)
+        state = 2;
     };
     auto make_item = [&](unsigned li, FRItem& it) {   // item li of this queue: band-major, the strips of a band neighbours
         if (li >= nitems) {
@@ -778,7 +789,12 @@ __device__ __forceinline__ void fr_chain_run(const FRArgs& a, const int lane, co
     pend.X = 0; pend.ys = 0; pend.nrows = 0; pend.P = 1; pend.interior = false; pend.done = false; pend.sf = a.src; pend.df = a.dst;
     // (one item per ticket: two / four neighbouring strips per ticket -- fewer draws -- measured 6 / 12 % SLOWER, tools/ablate_chain_misc.py:
     //  the strips of a band must be in flight together)
-    auto next_item = [&]() { make_item(draw(), pend); };
+    auto next_item = [&]() {
+        if (state == 1) take();   // (asked for in this trip, less than kLead steps ago: items barely longer than a trip)
+        state = 0;
+        make_item(ticket, pend);
+    };
+    ask();
     next_item();
     if (pend.done) return;               // (every wave draws its items + 1 tickets of every queue it visits: the host's accounting)
 
@@ -840,7 +856,7 @@ __device__ __forceinline__ void fr_chain_run(const FRArgs& a, const int lane, co
         dst[2] = *(const v4i*)(r_sf + off + 32);
         r_y += 2;
         r_off += 2 * sstep;
-        if (++ri == r_P) {
+        if (++ri == r_P) {   // (the prologue's RP - 1 requests stay inside the first item: P >= RP)
             if (!r_done) next_item();
             if (pend.done) {                         // past the last one: keep re-reading its last pair (cache hits, never used)
                 r_done = true;
@@ -924,8 +940,11 @@ __device__ __forceinline__ void fr_chain_run(const FRArgs& a, const int lane, co
     }
 
     for (;;) {
+        // the request cursor enters its next item in this trip, or within kLead steps of the next one (an item is at least a trip long)
+        if (state == 0 && !r_done && ri + RP + kLead >= r_P) ask();
 #pragma unroll
         for (int s = 0; s < RP; ++s) {
+            if (s == kLead && state == 1) take();
             request((s + RP - 1) % RP);
             const bool valid = oi <= o_P - NP;          // the window's NP pairs belong to one item
             const bool two = 2 * oi + 1 < o_nrows;      // ... and its second output row exists (odd band heights)
@@ -1566,8 +1585,11 @@ static int rows_launch(rcv_ctx* ctx, const View& s, const View& d, const int16_t
     if (src_yuyv == 0 && !sob && (dmask == 0 || chain_dual_ok) && (small_plan == 0 || kn.chain >= 1) && kn.band_rows == 0 && kn.chain != 0 && s.rows >= 64 &&
         ctx->cu_count == 256 && !ctx->fr_chain_off) {
         const int want_rows = kn.chain_rows > 0 ? (kn.chain_rows > 2048 ? 2048 : kn.chain_rows) : 32;   // (bmul < 2^32)
+        // rows of the shortest item: its row pairs must cover a trip of the kernel's loop, (item_rows + 1) / 2 + NP - 1 >= RP = NP + PP
+        // (the product's PP is 3; the measurement build's knob sets it)
+        const int item_rows = 2 * (kn.pp == 2 || kn.pp == 4 ? kn.pp : 3) + 1;
         int bpf = (s.rows + want_rows / 2) / want_rows;
-        bpf = bpf < 1 ? 1 : (bpf > s.rows / 8 ? s.rows / 8 : bpf);
+        bpf = bpf < 1 ? 1 : (bpf > s.rows / (item_rows + 1) ? s.rows / (item_rows + 1) : bpf);
         const unsigned long long nbands = (unsigned long long)s.n * bpf, nitems = 4 * ((nbands + 7) / 8) * a.nstrips;   // (bound on the items of the longest run, all of it quartered)
         const int cwpc = kn.wpc == 12 || kn.wpc == 4 || kn.wpc == 6 || kn.wpc == 10 ? kn.wpc : 8;   // (knob: waves per CU, sweeps)
         const unsigned waves = (unsigned)(ctx->cu_count / 8 * cwpc);   // per XCD: cu_count / 8 CUs x 8 waves
@@ -1616,10 +1638,10 @@ static int rows_launch(rcv_ctx* ctx, const View& s, const View& d, const int16_t
                 unsigned t1 = per_xcd / 8 < 8 ? per_xcd / 8 : 8, t2 = per_xcd / 16 < 4 ? per_xcd / 16 : 4;
                 if (kn.taper >= 0) t1 = (unsigned)kn.taper & 255u, t2 = (unsigned)kn.taper >> 8;
                 if (t1 + t2 > per_xcd / 2) t1 = t2 = 0;   // short runs: no taper
-                // an item needs >= 7 rows (more row pairs than the ring's prefetch depth): halves of bands of 14+, quarters of bands of 28+ rows
+                // an item needs item_rows (7) rows: halves of bands of 14+, quarters of bands of 28+ rows
                 const int br_min = s.rows / bpf;
-                if (br_min < 28) t2 = 0;
-                if (br_min < 14) t1 = 0;
+                if (br_min < 4 * item_rows) t2 = 0;
+                if (br_min < 2 * item_rows) t1 = 0;
                 a.tp1 = t1;
                 a.tp2 = t2;
             }
