@@ -53,8 +53,7 @@ __device__ __forceinline__ void static_for(F&& f)
     }
 }
 
-// Weights travel as kernel arguments and stay in SGPRs, two per 64-bit pair: v_pk_fma_f32 broadcasts either half of the pair
-// to both of its lanes (op_sel / op_sel_hi), so a weight costs one SGPR, not a {w, w} pair (49 pairs would not fit).
+// Weights travel as kernel arguments and stay in SGPRs, two per 64-bit pair.
 template <int KS, bool SEP>
 struct FWeights {
     f2 w2[((SEP ? KS : KS * KS) + 1) / 2];
@@ -63,14 +62,13 @@ struct FWeights {
                     // formed as floor(sum * 2^-shift + 0.5) (iscale = 2^-shift; every step exact in f32), then saturated
 };
 
-// d = fma({w, w}, x, acc) with w = half HALF of the uniform pair `wp`
-// (`half` is a compile-time constant after unrolling: the branch folds)
-__device__ __forceinline__ f2 pk_fma_w(int half, f2 wp, f2 x, f2 acc)
+// d = fma({w, w}, x, acc) with w = half `half` of the uniform pair `wp` (a compile-time constant after unrolling): two v_fma_f32 that read
+// the weight's SGPR.  (No packed f32 arithmetic in this library, see the Makefile.  What it costs here, 64 x 4K BGR, same run: dense 7x7 f32
+// 1.771 -> 2.973 ms, 7-tap Gaussian 0.893 -> 0.948 ms.)
+__device__ __forceinline__ f2 fma2_w(int half, f2 wp, f2 x, f2 acc)
 {
-    f2 d;
-    if (half == 0) asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel_hi:[0,1,1]" : "=v"(d) : "s"(wp), "v"(x), "v"(acc));
-    else asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,1,1]" : "=v"(d) : "s"(wp), "v"(x), "v"(acc));
-    return d;
+    const float w = half == 0 ? wp.x : wp.y;
+    return f2{__builtin_fmaf(w, x.x, acc.x), __builtin_fmaf(w, x.y, acc.y)};
 }
 
 // The NW window dwords of a thread as 16-byte loads (+ an 8- / 4-byte rest): the rows are 4-byte aligned, which is all a global load
@@ -172,12 +170,8 @@ __global__ __launch_bounds__(kBlock) void k_filter_f32_stream(View s, View d, FW
         }
     };
 
-    // The four samples of a thread ride in two packed-f32 pairs (samples 0,1 and 2,3): v_pk_fma_f32 performs two IEEE
-    // fmaf per instruction with the weight broadcast to both halves -- the same per-sample chain as the scalar oracle, at
-    // half the issue cost.  Sample j of tap kx reads p[j + kx*CH]; the pair {p[m], p[m+1]} is formed by the compiler
-    // (two v_mov_b32 when m is odd.  Round 6: written as vector shuffles of even-aligned pairs every odd pair is ONE v_pk_mov_b32 -- 960 -> 911
-    //  instructions in the 7-tap BGR instantiation -- and the launches were 1 % (7-tap Gaussian) to 6.5 % (dense 7x7 f32) SLOWER, same box, three
-    //  rotations: the packed move does not issue at the rate of a plain one.  Not kept; tools/ab_fs_variants.sh.)
+    // The samples of a thread are held as pairs (samples 0,1 and 2,3 ...), one v_fma_f32 per sample and tap -- the same per-sample chain as
+    // the scalar oracle.  Sample j of tap kx reads p[j + kx*CH].
     f2 acc[KS][NP];
 #pragma unroll
     for (int i = 0; i < KS; ++i)
@@ -205,7 +199,7 @@ __global__ __launch_bounds__(kBlock) void k_filter_f32_stream(View s, View d, FW
 #pragma unroll
             for (int kx = 0; kx < KS; ++kx) {
 #pragma unroll
-                for (int jj = 0; jj < NP; ++jj) h[jj] = pk_fma_w(kx & 1, W.w2[kx >> 1], f2{p[2 * jj + kx * CH], p[2 * jj + 1 + kx * CH]}, h[jj]);
+                for (int jj = 0; jj < NP; ++jj) h[jj] = fma2_w(kx & 1, W.w2[kx >> 1], f2{p[2 * jj + kx * CH], p[2 * jj + 1 + kx * CH]}, h[jj]);
                 if (RCV_FS_SCHED) __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -214,7 +208,7 @@ __global__ __launch_bounds__(kBlock) void k_filter_f32_stream(View s, View d, FW
             for (int ky = 0; ky < KS; ++ky) {
                 const int slot = ((RHO - ky + RAD) % KS + KS) % KS;
 #pragma unroll
-                for (int jj = 0; jj < NP; ++jj) acc[slot][jj] = pk_fma_w(ky & 1, W.w2[ky >> 1], h[jj], acc[slot][jj]);
+                for (int jj = 0; jj < NP; ++jj) acc[slot][jj] = fma2_w(ky & 1, W.w2[ky >> 1], h[jj], acc[slot][jj]);
             }
         } else {
             // dense: tap-major as well -- for one kx the KS output slots x NP pairs are independent accumulators (each still sees its own
@@ -226,7 +220,7 @@ __global__ __launch_bounds__(kBlock) void k_filter_f32_stream(View s, View d, FW
                     const int slot = ((RHO - ky + RAD) % KS + KS) % KS;
 #pragma unroll
                     for (int jj = 0; jj < NP; ++jj)
-                        acc[slot][jj] = pk_fma_w((ky * KS + kx) & 1, W.w2[(ky * KS + kx) >> 1], f2{p[2 * jj + kx * CH], p[2 * jj + 1 + kx * CH]}, acc[slot][jj]);
+                        acc[slot][jj] = fma2_w((ky * KS + kx) & 1, W.w2[(ky * KS + kx) >> 1], f2{p[2 * jj + kx * CH], p[2 * jj + 1 + kx * CH]}, acc[slot][jj]);
                 }
                 if (RCV_FS_SCHED) __builtin_amdgcn_sched_barrier(0);
             }
@@ -306,17 +300,15 @@ __global__ __launch_bounds__(kBlock) void k_filter_f32_stream(View s, View d, FW
 }
 
 // ---- the separable pass on ROW PAIRS (round 5) ---------------------------------------------------------------------------------
-// k_filter_f32_stream pairs ADJACENT SAMPLES of one row in a packed-f32 register: tap kx of the pair starting at sample m reads
-// {p[m + kx CH], p[m + 1 + kx CH]}, which for three channels is an even-aligned register pair only for every other kx -- the rest are
-// rebuilt with moves, and the converted window is per row.  Here the two halves of a pair are the SAME sample of two consecutive
-// rows: P2[b] = {row r byte b, row r + 1 byte b} (each half one v_cvt_f32_ubyteN), every tap index is an aligned pair, the
+// k_filter_f32_stream pairs ADJACENT SAMPLES of one row and converts its window per row.  Here the two halves of a pair are the SAME sample of two consecutive
+// rows: P2[b] = {row r byte b, row r + 1 byte b} (each half one v_cvt_f32_ubyteN), the
 // horizontal pass gives he = {h(r), h(r + 1)} per column, and the vertical pass accumulates OUTPUT row pairs (y, y + 1):
 //     acc(y, y + 1) += t[ky] * {h(y + ky - RAD), h(y + 1 + ky - RAD)}
-// -- the pair that starts on the row pair's first row is he itself, the one that starts a row earlier is ho = {previous he.y, he.x}
-// (one v_pk_mov per column and row pair).  Every output sees its taps in ky order (within a row pair: ho, one ky lower, before he),
+// -- the pair that starts on the row pair's first row is he itself, the one that starts a row earlier is ho = {previous he.y, he.x}.
+// Every output sees its taps in ky order (within a row pair: ho, one ky lower, before he),
 // each chain starts with a multiply (= fma(w, x, 0) for everything a u8 store can tell apart), so the result is the oracle's, bit for
-// bit.  RAD + 1 output pairs are in flight (static slots: the loop is unrolled by RAD + 1 row pairs).  Per sample: 3.25 conversions +
-// 2 x KS / 2 packed fma + 0.5 move + the store conversion -- 12.3 instructions for 7 taps of BGR against ~15.4.
+// bit.  RAD + 1 output pairs are in flight (static slots: the loop is unrolled by RAD + 1 row pairs).  Per sample: 3.25 conversions
+// + 2 x KS fma + the store conversion.
 template <int KS, int CH>
 __global__ __launch_bounds__(kBlock) void k_gauss_f32_pairs(View s, View d, FWeights<KS, true> W, int seg_rows, int gx, int gy, int nblocks, int blocks_per_xcd)
 {
@@ -365,7 +357,7 @@ __global__ __launch_bounds__(kBlock) void k_gauss_f32_pairs(View s, View d, FWei
 #pragma unroll
         for (int kx = 1; kx < KS; ++kx) {
 #pragma unroll
-            for (int j = 0; j < BPT; ++j) he[j] = pk_fma_w(kx & 1, W.w2[kx >> 1], P2[j + kx * CH], he[j]);
+            for (int j = 0; j < BPT; ++j) he[j] = fma2_w(kx & 1, W.w2[kx >> 1], P2[j + kx * CH], he[j]);
             __builtin_amdgcn_sched_barrier(0);   // (keeps the tap-major order: without it the compiler re-serialises the chains, +3 % at 7 taps)
         }
 #pragma unroll
@@ -383,12 +375,12 @@ __global__ __launch_bounds__(kBlock) void k_gauss_f32_pairs(View s, View d, FWei
             if (kyo >= 0 && kyo < KS) {
 #pragma unroll
                 for (int j = 0; j < BPT; ++j)
-                    acc[slot][j] = kyo == 0 ? ho[j] * f2{W.w2[0][0], W.w2[0][0]} : pk_fma_w(kyo & 1, W.w2[kyo >> 1], ho[j], acc[slot][j]);
+                    acc[slot][j] = kyo == 0 ? ho[j] * f2{W.w2[0][0], W.w2[0][0]} : fma2_w(kyo & 1, W.w2[kyo >> 1], ho[j], acc[slot][j]);
             }
             if (kye >= 0 && kye < KS) {
 #pragma unroll
                 for (int j = 0; j < BPT; ++j)
-                    acc[slot][j] = kye == 0 ? he[j] * f2{W.w2[0][0], W.w2[0][0]} : pk_fma_w(kye & 1, W.w2[kye >> 1], he[j], acc[slot][j]);
+                    acc[slot][j] = kye == 0 ? he[j] * f2{W.w2[0][0], W.w2[0][0]} : fma2_w(kye & 1, W.w2[kye >> 1], he[j], acc[slot][j]);
             }
             if (kyo == KS - 1 || kye == KS - 1) {   // this output pair is complete: rows y, y + 1
                 const int y = (kyo == KS - 1 ? R - 1 : R) - RAD;
@@ -471,9 +463,9 @@ int launch(rcv_ctx* ctx, const View& s, const View& d, const float* w, float del
         const int bpx = xcd ? (int)((nb + 7) / 8) : 0;
         const dim3 grid = xcd ? dim3((unsigned)bpx * 8u) : dim3(gx, gy, s.n);
         if constexpr (SEP && BPT == 8 && !RAG) {
-            // where it measures faster than the one-row kernel in its tap-major form (tools/ab_fs_variants.sh, same call, 64 x 4K BGR:
-            // 3 taps 0.640 against 0.665 ms; 5 / 7 taps equal; 11 taps 3.5 % slower; one channel never); RCV_GAUSS_ROWS=1 (tests)
-            // sends every shape here
+            // where it measures at least as fast as the one-row kernel on every shape (same process, medians: 3 taps of 64 x 4K BGR 0.736
+            // against 0.737 ms, 64 x 1080p BGR 0.198 / 0.200; 9 taps 1.375 / 1.230; one channel 3 ... 7 taps equal); RCV_GAUSS_ROWS=1
+            // (tests) sends every shape here
             const bool pairs = g_fs_pairs >= 0 ? g_fs_pairs != 0 : (rcv_knobs().gauss_rows == 1 || (CH == 3 && KS == 3));
             if (g_fs_lds > 65536u) {   // (measurement build: more than the default 64 KB of dynamic LDS needs the attribute)
                 (void)hipFuncSetAttribute((const void*)k_gauss_f32_pairs<KS, CH>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)g_fs_lds);

@@ -435,9 +435,9 @@ __device__ __forceinline__ void bilerp_bgrx_pair(const uint32_t (&p)[2][4], f2 f
     for (int k = 0; k < 2; ++k) {
         const f2 a0 = {ub<0>(p[k][0]), ub<1>(p[k][0])}, a1 = {ub<0>(p[k][1]), ub<1>(p[k][1])};
         const f2 b0 = {ub<0>(p[k][2]), ub<1>(p[k][2])}, b1 = {ub<0>(p[k][3]), ub<1>(p[k][3])};
-        const f2 top = k ? pk_fma_bc<1>(fxp, a1 - a0, a0) : pk_fma_bc<0>(fxp, a1 - a0, a0);
-        const f2 bot = k ? pk_fma_bc<1>(fxp, b1 - b0, b0) : pk_fma_bc<0>(fxp, b1 - b0, b0);
-        v01[k] = (k ? pk_fma_bc<1>(fyp, bot - top, top) : pk_fma_bc<0>(fyp, bot - top, top)) + half2;
+        const f2 top = k ? fma2_bc<1>(fxp, a1 - a0, a0) : fma2_bc<0>(fxp, a1 - a0, a0);
+        const f2 bot = k ? fma2_bc<1>(fxp, b1 - b0, b0) : fma2_bc<0>(fxp, b1 - b0, b0);
+        v01[k] = (k ? fma2_bc<1>(fyp, bot - top, top) : fma2_bc<0>(fyp, bot - top, top)) + half2;
     }
     const f2 c00 = {ub<2>(p[0][0]), ub<2>(p[1][0])}, c01 = {ub<2>(p[0][1]), ub<2>(p[1][1])};
     const f2 c10 = {ub<2>(p[0][2]), ub<2>(p[1][2])}, c11 = {ub<2>(p[0][3]), ub<2>(p[1][3])};
@@ -672,7 +672,7 @@ __global__ __launch_bounds__(kBlock) void k_warp_affine_lds(View s, View d, Affi
                     const int r = 4 * h + i;
                     const uint32_t a = *(lcu)(uintptr_t)(la[B][r]), b = *(lcu)(uintptr_t)(lb[B][r]);
                     const f2 p0 = {ub<0>(a), ub<0>(b)}, p1 = {ub<1>(a), ub<1>(b)};
-                    const f2 tb2 = (r & 1) ? pk_fma_bc<1>(fxp[r >> 1], p1 - p0, p0) : pk_fma_bc<0>(fxp[r >> 1], p1 - p0, p0);
+                    const f2 tb2 = (r & 1) ? fma2_bc<1>(fxp[r >> 1], p1 - p0, p0) : fma2_bc<0>(fxp[r >> 1], p1 - p0, p0);
                     t[i] = trunc_u32(fmaf(fyp[r >> 1][r & 1], tb2.y - tb2.x, tb2.x) + 0.5f);   // every tap inside the source: an integer in [0, 255]
                 }
             } else {
@@ -760,7 +760,7 @@ __global__ __launch_bounds__(kBlock) void k_warp_affine_lds(View s, View d, Affi
 // frames, 24 % of the HBM roofline).  A one-channel patch pixel fills one byte of its LDS dword; this kernel fills all four with
 // the SAME pixel of four consecutive frames {f0 f1 f2 f3}: a chunk's four dwords (one per frame, 4 pixels each) go through a
 // 4 x 4 byte transpose (8 v_perm) into one ds_write_b128, one ds_read_b64 returns a tap pair of all four frames, the coordinates /
-// weights are shared anyway, the lerps of two frames ride in one packed-f32 operation, the results of four frames go through ONE
+// weights are shared anyway, the results of four frames go through ONE
 // quad transpose (as dwords {f0 f1 f2 f3}) and a byte transpose back.  A quarter of the LDS instructions and barriers per frame,
 // the same f32 operations per pixel in the same order.  Aligned sources only (base, step, frame stride multiples of 4: a chunk is
 // one aligned dword); everything else stays on k_warp_affine_lds<1>.
@@ -907,9 +907,9 @@ __global__ __launch_bounds__(kBlock) void k_warp_gray_lds4(View s, View d, Affin
                 // v = fma(fy, bot - top, top) + 0.5 -- k_warp_affine_gray's operations, two frames per packed instruction
                 const f2 p00 = {ub<0>(a0), ub<1>(a0)}, p01 = {ub<0>(a1), ub<1>(a1)}, p10 = {ub<0>(b0), ub<1>(b0)}, p11 = {ub<0>(b1), ub<1>(b1)};
                 const f2 q00 = {ub<2>(a0), ub<3>(a0)}, q01 = {ub<2>(a1), ub<3>(a1)}, q10 = {ub<2>(b0), ub<3>(b0)}, q11 = {ub<2>(b1), ub<3>(b1)};
-                const f2 top = pk_fma_bc<0>(fxy[r], p01 - p00, p00), bot = pk_fma_bc<0>(fxy[r], p11 - p10, p10);
-                const f2 tpq = pk_fma_bc<0>(fxy[r], q01 - q00, q00), btq = pk_fma_bc<0>(fxy[r], q11 - q10, q10);
-                const f2 v01 = pk_fma_bc<1>(fxy[r], bot - top, top) + half2, v23 = pk_fma_bc<1>(fxy[r], btq - tpq, tpq) + half2;
+                const f2 top = fma2_bc<0>(fxy[r], p01 - p00, p00), bot = fma2_bc<0>(fxy[r], p11 - p10, p10);
+                const f2 tpq = fma2_bc<0>(fxy[r], q01 - q00, q00), btq = fma2_bc<0>(fxy[r], q11 - q10, q10);
+                const f2 v01 = fma2_bc<1>(fxy[r], bot - top, top) + half2, v23 = fma2_bc<1>(fxy[r], btq - tpq, tpq) + half2;
                 uint32_t px = pack_floor3(v01.x, v01.y, v23.x);
                 asm("v_cvt_u32_f32_sdwa %0, %1 dst_sel:BYTE_3 dst_unused:UNUSED_PRESERVE src0_sel:DWORD" : "+v"(px) : "v"(v23.y));
                 w[i] = px;
@@ -966,8 +966,8 @@ __global__ __launch_bounds__(kBlock) void k_warp_gray_lds4(View s, View d, Affin
 
 // One-channel images: the scheme of k_warp_affine_bgr with 2-byte tap pairs.  One thread per output column and kWarpRows
 // rows; a wave whose taps all lie inside the source fetches each tap pair as the ALIGNED 8 bytes that contain it (one dwordx2
-// per source row: 16 tap loads in flight per lane), shifts it into place with v_alignbyte, lerps top and bottom rows as one
-// packed-f32 pair, and after a quad transpose every lane stores the 4 pixels of one row as a dword.  Waves that touch the
+// per source row: 16 tap loads in flight per lane), shifts it into place with v_alignbyte, lerps top and bottom rows as
+// a pair, and after a quad transpose every lane stores the 4 pixels of one row as a dword.  Waves that touch the
 // border run warp_px<1> per pixel (same f32 operations, same order).
 __device__ __forceinline__ void warp_gray_frame(const View& s, const View& d, const Affine& A, const int frame, const int x, const int ybase)
 {
@@ -1008,7 +1008,7 @@ __device__ __forceinline__ void warp_gray_frame(const View& s, const View& d, co
             const uint32_t a = __builtin_amdgcn_alignbyte(ta[r].b, ta[r].a, sh[r]), b = __builtin_amdgcn_alignbyte(tb[r].b, tb[r].a, shb[r]);
             // {top, bottom} as one packed pair: fma(fx, p01 - p00, p00), then v = fma(fy, bot - top, top), floor(v + 0.5)
             const f2 p0 = {ub<0>(a), ub<0>(b)}, p1 = {ub<1>(a), ub<1>(b)};
-            const f2 tb2 = pk_fma_bc<0>(fxy[r], p1 - p0, p0);
+            const f2 tb2 = fma2_bc<0>(fxy[r], p1 - p0, p0);
             px[r] = trunc_u32(fmaf(fxy[r].y, tb2.y - tb2.x, tb2.x) + 0.5f);   // interior: an integer in [0, 255]
         }
     } else {
@@ -1041,7 +1041,7 @@ __global__ __launch_bounds__(kBlock) void k_warp_affine_gray(View s, View d, Aff
 
 // ---- bilinear resize, BGR, any scale: the register scheme of k_warp_affine_bgr ------------------------------------------
 // One thread per output column and kRszRows consecutive output rows: x0 and fx are computed once, every row costs two
-// aligned 12-byte tap windows (all in flight together), packed-f32 lerps, and four lanes share a 12-byte store.  A wave
+// aligned 12-byte tap windows (all in flight together), pairwise lerps, and four lanes share a 12-byte store.  A wave
 // whose lanes all have x0 <= cols-4 (the whole tap window inside the row) takes this path; the few waves at the right
 // edge run resize_px<3> per pixel.  Same f32 operations in the same order as resize_px<3>.
 constexpr int kRszRows = 4;
@@ -1156,7 +1156,7 @@ __global__ __launch_bounds__(kBlock) void k_resize_gray(View s, View d, float sc
         for (int r = 0; r < kRszRows; ++r) {
             const uint32_t a = __builtin_amdgcn_alignbyte(ta[r].b, ta[r].a, sha[r]), b = __builtin_amdgcn_alignbyte(tb[r].b, tb[r].a, shb[r]);
             const f2 p0 = {ub<0>(a), ub<0>(b)}, p1 = {ub<1>(a), ub<1>(b)};
-            const f2 tb2 = pk_fma_bc<0>(f2{fx, fy[r]}, p1 - p0, p0);          // {top, bottom}: fma(fx, p01 - p00, p00)
+            const f2 tb2 = fma2_bc<0>(f2{fx, fy[r]}, p1 - p0, p0);          // {top, bottom}: fma(fx, p01 - p00, p00)
             px[r] = trunc_u32(fmaf(fy[r], tb2.y - tb2.x, tb2.x) + 0.5f);   // an integer in [0, 255]
         }
         static_assert(kRszRows == 4, "one quad transpose per thread");
@@ -1438,7 +1438,7 @@ __global__ __launch_bounds__(kBlock) void k_warp_f32_lds(View s, View d, Affine 
         for (int r = 0; r < kWarpRows; ++r) {
             const lcf pa = (lcf)(uintptr_t)(la[B][r]), pb = (lcf)(uintptr_t)(la[B][r] + (unsigned)pitch);
             const f2 p0 = {pa[0], pb[0]}, p1 = {pa[1], pb[1]};
-            const f2 tb = pk_fma_bc<0>(fxy[r], p1 - p0, p0);                     // {top, bottom}: fma(fx, p01 - p00, p00), fma(fx, p11 - p10, p10)
+            const f2 tb = fma2_bc<0>(fxy[r], p1 - p0, p0);                     // {top, bottom}: fma(fx, p01 - p00, p00), fma(fx, p11 - p10, p10)
             const float v = fmaf(fxy[r].y, tb.y - tb.x, tb.x);
             if constexpr (INNER) {
                 asm volatile("" : "+v"(so[r]));

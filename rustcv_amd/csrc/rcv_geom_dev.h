@@ -1,5 +1,5 @@
 // rcv_geom_dev.h -- device helpers shared by the geometry kernels (rcv_geom.hip: resize / warpAffine; rcv_warp_resize.hip: the
-// fused warpAffine -> down-scale launches): the byte-granular reference formulation of one warped pixel, the packed-f32 bilinear
+// fused warpAffine -> down-scale launches): the byte-granular reference formulation of one warped pixel, the bilinear
 // sample of a BGR pixel from its tap dwords, the XCD-aware tile order.  f32 evaluation order is fixed and spelled out op by op
 // (SURVEY.md 8-A == oracle/rcv_oracle.c orc_resize / orc_warp_affine); built with -ffp-contract=off.
 #pragma once
@@ -103,20 +103,18 @@ __device__ __forceinline__ float ub(uint32_t v)
 // Bilinear sample of one BGR pixel from its two tap dwords per row {b0 g0 r0 b1 | g1 r1 . .} (upper row a, lower row b),
 // packed {b, g, r, 0}.  The f32 operations and their order are those of warp_px<3> / resize_px<3>: per channel
 // top = fma(fx, p01 - p00, p00), bot = fma(fx, p11 - p10, p10), v = fma(fy, bot - top, top), floor(v + 0.5).  Channels 0 and 1
-// ride in packed-f32 pairs, channel 2 pairs its top and bottom row (v_pk_add / v_pk_fma: two IEEE operations per
-// instruction, bit-identical to the scalar ops).  All taps must be valid (interior), so the result is an exact integer in
+// are written as pairs, channel 2 pairs its top and bottom row (two scalar f32 operations each: no packed f32 arithmetic in this
+// library, see the Makefile).  All taps must be valid (interior), so the result is an exact integer in
 // [0, 255] and v_cvt_pk_u8_f32 converts, saturates and packs it.
 // PIN = true pins each byte conversion to one v_cvt_f32_ubyteN (fewer instructions: -2 % in the 8-row warp / 4-row resize
 // kernels); the fused down-scale kernel, which interleaves four pixels, schedules better with the compiler's own choice.
-// d = fma({w, w}, a, b) with w = the low (HI = 0) or the high (HI = 1) half of the register pair wp: op_sel broadcasts the
-// half, so the {fx, fy} pair the coordinate arithmetic leaves behind feeds all four lerps without a v_mov to duplicate it
+// d = fma({w, w}, a, b) with w = the low (HI = 0) or the high (HI = 1) half of the pair wp: the {fx, fy} pair the coordinate arithmetic
+// leaves behind feeds all four lerps
 template <int HI>
-__device__ __forceinline__ f2 pk_fma_bc(f2 wp, f2 a, f2 b)
+__device__ __forceinline__ f2 fma2_bc(f2 wp, f2 a, f2 b)
 {
-    f2 d;
-    if constexpr (HI == 0) asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel_hi:[0,1,1]" : "=v"(d) : "v"(wp), "v"(a), "v"(b));
-    else asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,1,1]" : "=v"(d) : "v"(wp), "v"(a), "v"(b));
-    return d;
+    const float w = HI == 0 ? wp.x : wp.y;
+    return f2{__builtin_fmaf(w, a.x, b.x), __builtin_fmaf(w, a.y, b.y)};
 }
 
 // {floor(b), floor(g), floor(r), 0} of three values in [0, 256): v_cvt_u32_f32 truncates (= floor for these non-negative values)
@@ -154,10 +152,10 @@ __device__ __forceinline__ uint32_t bilerp_bgr(uint32_t alo, uint32_t ahi, uint3
         c0 = f2{(float)((alo >> 16) & 0xff), (float)((blo >> 16) & 0xff)}; c1 = f2{(float)((ahi >> 8) & 0xff), (float)((bhi >> 8) & 0xff)};
     }
     const f2 half2 = {0.5f, 0.5f};
-    const f2 top = pk_fma_bc<0>(fxy, a1 - a0, a0);
-    const f2 bot = pk_fma_bc<0>(fxy, b1 - b0, b0);
-    const f2 tb2 = pk_fma_bc<0>(fxy, c1 - c0, c0);
-    const f2 v01 = pk_fma_bc<1>(fxy, bot - top, top) + half2;
+    const f2 top = fma2_bc<0>(fxy, a1 - a0, a0);
+    const f2 bot = fma2_bc<0>(fxy, b1 - b0, b0);
+    const f2 tb2 = fma2_bc<0>(fxy, c1 - c0, c0);
+    const f2 v01 = fma2_bc<1>(fxy, bot - top, top) + half2;
     const float v2 = fmaf(fxy.y, tb2.y - tb2.x, tb2.x) + 0.5f;
     return pack_floor3(v01.x, v01.y, v2);
 }   // output rows per thread: fewer, longer-lived workgroups and 16 tap loads in flight per lane

@@ -48,9 +48,9 @@ __device__ __forceinline__ float shl1f(float v) { return __builtin_bit_cast(floa
 __device__ __forceinline__ int mad24(int a, int b, int c) { return __mul24(a, b) + c; }   // v_mad_i32_i24: |Ix|, |Iy| <= 1020
 
 // Blocks up to 4: block^2 * 1020^2 < 2^24, so the window sums (and every partial sum on the way) are integers f32 holds exactly.
-// The gradients of a row are converted on the way in and on the way out and the sums run on packed f32 -- two pixels per
-// instruction, pixels j and j+4 of the lane in one pair -- already in the form the response arithmetic wants (block 3, 4K batch
-// of 64: 0.75 -> 0.66 ms from BGR, 0.64 -> 0.54 ms from gray; the i32 form stays for blocks 5..7).
+// The gradients of a row are converted on the way in and on the way out and the sums run on f32,
+// pixels j and j+4 of the lane as a pair, already in the form the response arithmetic wants (block 3, 4K batch of 64, from BGR: 0.642 ms,
+// with packed f32 arithmetic 0.620; in i32 0.75; the i32 form stays for blocks 5..7).
 template <int B>
 struct WindowF32 {
     static constexpr int AN = B / 2, RT = B - 1 - AN;

@@ -5,7 +5,7 @@
 // One WAVE owns a strip of 496 px (62 lanes x 8 px; lanes 0 / 63 carry halo only) and walks down a row segment.
 // Per source row a lane loads its 8 BGR pixels (3 x 8 B), converts to gray, and every stage pulls the one neighbour
 // value it needs from the adjacent lane with a DPP wave shift:
-//     gray      needs g[x-1], g[x+1]            (Sobel: packed f32 on aligned shapes, packed i16 as in rcv_sobel_rows.hip elsewhere)
+//     gray      needs g[x-1], g[x+1]            (Sobel: f32 on aligned shapes, packed i16 as in rcv_sobel_rows.hip elsewhere)
 //     box 2x2   needs P[x-1]  (P = Ix^2, IxIy, Iy^2 ; window offsets -1..0, anchor = blockSize/2 = 1)
 //     NMS 3x3   needs r[x-1], r[x+1]
 // Vertical neighbours are earlier rows kept in registers (2 rows of Sobel parts, 1 row of horizontal box sums,
@@ -14,9 +14,8 @@
 // is negated on the mirrored row (a mirrored Sobel flips the sign of dy); the left border P(-1) := P(1) is a lane
 // fix-up; response values outside the image are -inf for the NMS.  f32 ops follow the oracle's order exactly
 // (six separate IEEE ops, -ffp-contract=off).
-// Round 6, from the ISA: 192 -> ~165 vector instructions per row.  The packed-f32 stages work on pairs {pixel j, pixel j + 4};
-// pairs 0 and 3 are kept with their halves swapped (op_sel where they are plain operands) so that the strip-end neighbour pairs are those
-// registers after one in-place DPP move; aligned shapes address their rows through buffer resources (row offset in the instruction's scalar
+// The f32 stages work on pairs {pixel j, pixel j + 4}; pairs 0 and 3 are kept with their halves swapped so that the strip-end neighbour pairs
+// are those registers after one DPP move; aligned shapes address their rows through buffer resources (row offset in the instruction's scalar
 // offset: no vector address arithmetic); the NMS takes column maxima first and forms the mask bytes from the sign of centre - maximum.
 // RAG instantiation: any width >= 8 and any alignment (Mat::new gives step = cols * channels: odd widths mean byte-aligned
 // rows): unaligned vector loads / stores, the lane with the row's last, partial run rebuilds its 8 logical gray pixels --
@@ -97,7 +96,7 @@ __device__ __forceinline__ float shr1f(float v) { return __builtin_bit_cast(floa
 __device__ __forceinline__ float shl1f(float v) { return __builtin_bit_cast(float, shl1(__builtin_bit_cast(uint32_t, v))); }
 
 // The NMS maxima as the instructions themselves: through fmaxf the compiler first canonicalises every operand it cannot prove quiet (a
-// v_max_f32 x, x per pixel: values extracted from packed-f32 results, DPP moves); the hardware maxima give the same result for the values
+// v_max_f32 x, x per pixel: values extracted from pairs, DPP moves); the hardware maxima give the same result for the values
 // that occur here (finite responses and -inf) without it.  Round 4, from the ISA: 1 of 29 instructions per pixel.
 __device__ __forceinline__ float vmax2(float a, float b)
 {
@@ -112,11 +111,20 @@ __device__ __forceinline__ float vmax3(float a, float b, float c)
     return d;
 }
 
-// Packed-f32 operations that read one operand with its halves SWAPPED (op_sel), for the pairs kept as {pixel j + 4, pixel j}: round 6.  A lane's
-// pairs are {pixel j, pixel j + 4}; the neighbour pair of j = 0 is {pixel -1, pixel 3} = {lane-1's pixel 7, own pixel 3}.  With pair 3 kept
-// SWAPPED, {pixel 7, pixel 3}, that neighbour pair is pair 3 itself after ONE in-place DPP move of its low half -- no copy of pixel 3 into
-// a second register pair (the compiler, given plain vector code, un-swaps the pair and copies).  The swap costs nothing where pair 3 is an
-// ordinary operand: op_sel picks the halves.  Same for pair 0 = {pixel 4, pixel 0} and the neighbour pair {pixel 4, pixel 8} of j = 3.
+// Operations that read an operand with its halves SWAPPED, for the pairs kept as {pixel j + 4, pixel j}.  A lane's pairs are {pixel j,
+// pixel j + 4}; the neighbour pair of j = 0 is {pixel -1, pixel 3} = {lane-1's pixel 7, own pixel 3}.  With pair 3 kept SWAPPED, {pixel 7,
+// pixel 3}, that neighbour pair is pair 3 itself after ONE DPP move of its low half.  Same for pair 0 = {pixel 4, pixel 0} and the neighbour
+// pair {pixel 4, pixel 8} of j = 3.
+#ifdef RCV_NO_PACKED_F32
+// What the library is built with (see the Makefile): two scalar operations each.  64 x 4K, BGR -> mask: 0.453 ms against 0.444 with the
+// packed forms, from YUYV 0.636 / 0.580, from gray 0.364 / 0.351, same run.
+__device__ __forceinline__ f2 pk_add_bs(f2 a, f2 b) { return f2{a.x + b.y, a.y + b.x}; }
+__device__ __forceinline__ f2 pk_sub_bs(f2 a, f2 b) { return f2{a.x - b.y, a.y - b.x}; }
+__device__ __forceinline__ f2 pk_sub_as(f2 a, f2 b) { return f2{a.y - b.x, a.x - b.y}; }
+__device__ __forceinline__ f2 pk_fma2_as(f2 a, f2 c) { return f2{__builtin_fmaf(a.y, 2.0f, c.x), __builtin_fmaf(a.x, 2.0f, c.y)}; }
+__device__ __forceinline__ f2 pk_mul_ss(f2 a, f2 b) { return f2{a.y * b.y, a.x * b.x}; }
+#else
+// In no library: the row loop that tests/test_isa_waits.py compiles without the Makefile's flags and counts these instructions in.
 __device__ __forceinline__ f2 pk_add_bs(f2 a, f2 b)   // {a.x + b.y, a.y + b.x}
 {
     f2 d;
@@ -147,6 +155,7 @@ __device__ __forceinline__ f2 pk_mul_ss(f2 a, f2 b)   // {a.y * b.y, a.x * b.x}
     asm("v_pk_mul_f32 %0, %1, %2 op_sel:[1,1] op_sel_hi:[0,0]" : "=v"(d) : "v"(a), "v"(b));
     return d;
 }
+#endif
 
 // byte 2 of a dword as f32 in ONE instruction (as C the compiler pulls the conversion through the Sobel's additions and does those in integer)
 __device__ __forceinline__ float cvb2(uint32_t w)
@@ -241,8 +250,7 @@ __global__ __launch_bounds__(64 * kWPB) RCV_HF_OCC_ATTR void k_harris_fused(HArg
     const __amdgpu_buffer_rsrc_t rrs = __builtin_amdgcn_make_buffer_rsrc((void*)rf, 0, 0xffffffff, kRsrc);
     const uint32_t sstep32 = (uint32_t)a.sstep, mstep32 = (uint32_t)a.mstep, rstep32 = (uint32_t)a.rstep;
     constexpr bool TQ = !GRAY && !RAG;   // gray values stay one per dword (byte 2), see feed
-    // the Sobel stage in packed f32 (mask-only launches: with the response the 16 more registers cost the third wave per SIMD); same box,
-    // same run, 64 x 4K: 0.4984-0.5012 ms against 0.5148-0.5189 with the packed-i16 Sobel
+    // the Sobel stage in f32: the gradients come out in the form the products want, without the packed-i16 Sobel's byte permutes and conversions
     // (round 6: a one-channel source too -- its eight pixels are the bytes of the two source dwords, v_cvt_f32_ubyte0..3 reads them in place)
     constexpr bool FSOB = (TQ || (GRAY && !RAG && RCV_HF_FSOB_GRAY)) && (!WANT_RESP || RCV_HF_FSOB_RESP) && RCV_HF_FSOB;
     const uint32_t sx = (uint32_t)((GRAY ? 1 : (YUYV ? 2 : 3)) * xc), mx = (uint32_t)max(x, 0);
@@ -280,10 +288,10 @@ __global__ __launch_bounds__(64 * kWPB) RCV_HF_OCC_ATTR void k_harris_fused(HArg
 
     // ---- pipeline state --------------------------------------------------------------------------------------
     uint32_t h1a[4], h1b[4], h2a[4], h2b[4];      // Sobel horizontal parts of gray rows v-2, v-1 (packed i16 pairs)
-    f2 f1a[4], f1b[4], f2a[4], f2b[4];            // ... the same as packed f32 pairs {pixel j, pixel j + 4} (FSOB)
+    f2 f1a[4], f1b[4], f2a[4], f2b[4];            // ... the same as f32 pairs {pixel j, pixel j + 4} (FSOB)
     f2 hsxx[4], hsxy[4], hsyy[4];                 // horizontal box sums of product row u-1 -- kept in f32: every product
                                                   // (<= 1020^2) and every 2x2 sum (< 2^24) is an exactly representable
-                                                  // integer, so f32 adds/muls are exact and can use the packed f32 ALU
+                                                  // integer, so f32 adds/muls are exact
     float ra[8], rb[8];                           // NMS: responses of rows u-2, u-1 (outside the image: -inf)
     int cand_b = 0;                               // ... and whether row u-1 holds a pixel >= thr_up (wave-uniform; an integer: as a bool it lived as a lane mask)
     // aligned shapes: the mask row formed at the end of one feed is stored after the Sobel stage of the NEXT one.  The wait for the next row
@@ -362,7 +370,7 @@ __global__ __launch_bounds__(64 * kWPB) RCV_HF_OCC_ATTR void k_harris_fused(HArg
                 }
             }
             if constexpr (FSOB) {
-                // Round 4: the Sobel in PACKED F32 on the pairs {pixel j, pixel j + 4} the later stages use anyway.  v_cvt_f32_ubyte2 takes
+                // Round 4: the Sobel in F32 on the pairs {pixel j, pixel j + 4} the later stages use anyway.  v_cvt_f32_ubyte2 takes
                 // the gray value straight out of byte 2 of its dword (one instruction per value), every intermediate is a small integer, so
                 // the f32 arithmetic is exact and Ix, Iy come out as the SAME f32 values the integer path converts to -- without its nine
                 // byte permutes and sixteen i16 -> f32 conversions.
@@ -442,7 +450,7 @@ __global__ __launch_bounds__(64 * kWPB) RCV_HF_OCC_ATTR void k_harris_fused(HArg
         const int u = v - 1;
         const bool mirrored = (unsigned)u >= (unsigned)a.rows;  // I(u) was formed from a vertically mirrored window: dy changes sign
         constexpr bool kLimRow = !WANT_RESP && !RAG && RCV_HF_LIMROW;
-        // f32 stages on PACKED pairs {pixel j, pixel j+4} (v_pk_mul/add_f32): with this pairing the horizontal neighbour
+        // f32 stages on pairs {pixel j, pixel j+4}: with this pairing the horizontal neighbour
         // P(x-1) of a pair is simply the previous pair register (j >= 1) -- pairing adjacent pixels {2j, 2j+1} instead leaves
         // every neighbour pair {2j-1, 2j} straddling two registers, and the compiler rebuilds it with ~3 v_mov per pixel
         f2 ix2[4], iy2[4];

@@ -107,7 +107,7 @@ def main():
         return float(f.value)
 
     def record(name, cfg, n, out_px, bpp, fn, note="", cpu=None, valu=None):
-        """valu = VALU instructions per output pixel the op's arithmetic needs at least (packed FMAs count as one): the row then
+        """valu = VALU instructions per output pixel the op's arithmetic needs at least: the row then
         carries its VALU roofline -- n * px * valu / (1024 SIMDs x 16 lanes per cycle x measured clock) / measured time"""
         if a.only and a.only.replace("_", " ") not in name + " @ " + cfg:   # "--only Sobel_3x3_->_dx,dy_i16_@_4K": op and config
             return
@@ -208,16 +208,16 @@ def main():
     record("filter2D 7x7 i8 (>>6)", "4K batch=64", s.n, 3840 * 2160, 6, lambda: device.filter2d(s, d, k7, shift=6))
     kf = (k7.astype(np.float32) / 64.0)
     record("filter2D 7x7 f32", "4K batch=64", s.n, 3840 * 2160, 6, lambda: device.filter2d(s, d, kf, delta=0.0),
-           note="VALU-bound by construction (49 dependent fmaf per sample), reported for completeness", valu=147 / 2)   # 3 x 49 FMA per px, two per v_pk_fma_f32
+           note="VALU-bound by construction (49 dependent fmaf per sample), reported for completeness", valu=147)   # 3 x 49 FMA per px
     record("GaussianBlur 7x7 (sigma=0)", "4K batch=64", s.n, 3840 * 2160, 6, lambda: device.gaussian_blur(s, d, 7, 0.0))
     record("GaussianBlur 7x7 (sigma=1.5)", "4K batch=64", s.n, 3840 * 2160, 6, lambda: device.gaussian_blur(s, d, 7, 1.5),
-           note="f32 separable path, 14 fmaf per sample", valu=42 / 2)
+           note="f32 separable path, 14 fmaf per sample", valu=42)
     # ---- config 5: Harris pipeline on 4K BGR, 64 frames per GPU ----------------------------------------------
     m = B(64, 2160, 3840, 1)
     device.synth(s, 1, SEED + 5, 0)
     record("Harris pipeline (BGR->mask)", "4K batch=64/GPU", s.n, 3840 * 2160, 4, lambda: device.harris_pipeline(s, m, None, 2, 0.04, 1e-4),
-           cpu=lambda: cpu_time(lambda orc: orc.harris_pipeline(np.zeros((2160, 3840, 3), np.uint8), 2, 0.04, 1e-4), 3840 * 2160),
-           valu=23)   # VALU instructions per pixel of the kernel as built (rocprofv3 SQ_INSTS_VALU 1.9e8 per launch, round 6; round 4: 28, round 2: 32)
+           cpu=lambda: cpu_time(lambda orc: orc.harris_pipeline(np.zeros((2160, 3840, 3), np.uint8), 2, 0.04, 1e-4), 3840 * 2160))   # (no VALU figure: 37 instructions per pixel, rocprofv3 SQ_INSTS_VALU
+    #      1.55e8 per 32-frame launch, issue at 3.3 cycles each -- conversions, moves, adds and maxima take less than the four of the model above)
     yq = B(64, 2160, 3840, 2)
     device.synth(yq, 2, SEED + 5, 0)
     record("Harris pipeline from a YUYV source (config 5 [or YUYV])", "4K batch=64/GPU", yq.n, 3840 * 2160, 3,
@@ -255,7 +255,8 @@ def main():
     device.synth(s, 0, SEED + 4, 0)
     M = rot_matrix(7.0, 7680 / 2, 4320 / 2, 13.25, -8.5)
     frac = warp_touched_fraction(M.astype(np.float64), 4320, 7680, 4320, 7680) if not a.only or "warpAffine bil" in a.only.replace("_", " ") or "GRAY" in a.only or "f32" in a.only else 1.0
-    record("warpAffine bilinear (rot 7deg)", "8K batch=32/GPU", s.n, 7680 * 4320, 3 + 3 * frac, lambda: device.warp_affine(s, d, M), valu=32,
+    record("warpAffine bilinear (rot 7deg)", "8K batch=32/GPU", s.n, 7680 * 4320, 3 + 3 * frac, lambda: device.warp_affine(s, d, M), valu=44,   # (SQ_INSTS_VALU 7.39e8 per launch)
+          
            note=f"3 B written per output px + 3 B per DISTINCT in-bounds source px touched ({frac:.4f} per output px, counted on the host; upper bound 6)",
            cpu=lambda: cpu_time(lambda orc: orc.warp_affine(np.zeros((4320, 7680, 3), np.uint8), M, 4320, 7680), 7680 * 4320, 6.0))
     d.free()
@@ -265,7 +266,7 @@ def main():
     sg.free(); dg.free()
     d = B(32, 1080, 1920, 3)
     record("warpAffine + resize 8K -> 1080p FUSED (next row f1)", "8K batch=32/GPU", s.n, 1920 * 1080, 30,
-           lambda: device.warp_affine_resize(s, d, M, 4320, 7680), valu=202,   # (k_warp_resize_stage, SQ_INSTS_VALU 2.09e8 per launch: ~160 in the frame loop + plans + border tiles; the gather kernel: 278)
+           lambda: device.warp_affine_resize(s, d, M, 4320, 7680), valu=230,   # (k_warp_resize_stage, SQ_INSTS_VALU 2.39e8 per launch)
            note="30 B per OUTPUT px: the centre 2x2 warped pixels of each 4x4 block tap a 3x3 source block (27 B) + 3 B written; "
                 "the unfused pair moves 6 B/px of 8K intermediate on top")
     d2 = B(32, 2880, 5120, 3)

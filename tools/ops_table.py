@@ -36,5 +36,5 @@ if len(sys.argv) <= 1:
     with open(os.path.join(ROOT, "profiles", "ops_table.md"), "w") as f:
         f.write("One MI355X, device-resident batches, sustained clocks (`python tools/bench_ops.py --cpu`; raw data: `ops_bench.json`).\n"
                 "Algorithmic bytes per pixel as DESIGN_HISTORY.md section 4 states them; launch-bound rows carry no roofline figure.  VALU roofline: the\n"
-                "op's VALU instructions per pixel (packed FMAs count once) x pixels / (1024 SIMDs x 16 lanes per cycle x the shader clock\n"
+                "op's VALU instructions per pixel x pixels / (1024 SIMDs x 16 lanes per cycle x the shader clock\n"
                 "measured under that op) / measured time -- min(HBM, VALU) is the bound of a row.\n\n" + text)

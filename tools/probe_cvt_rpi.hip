@@ -1,5 +1,5 @@
 // Does v_cvt_rpi_i32_f32 (documented as floor(x + 0.5)) equal floor(fl32(x + 0.5)) -- the reference's rounding -- for every
-// float in [0, 256)?  Exhaustive over the bit patterns 0 .. 0x43800000.   hipcc --offload-arch=gfx950 -O2 -o probe_cvt_rpi probe_cvt_rpi.hip
+// float in [0, 256)?  Exhaustive over the bit patterns 0 .. 0x43800000.   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -o probe_cvt_rpi probe_cvt_rpi.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

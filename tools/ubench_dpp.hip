@@ -1,7 +1,7 @@
 // tools/ubench_dpp.hip -- (round 6) what a DPP move costs on gfx950 by kind: plain v_mov_b32, row_shr:1, wave_shr:1, wave_shl:1 (the Harris / Sobel windows use the
-// wave-wide shifts: nine per row of the fused Harris kernel), and the packed-f32 ops beside them.  One wave per SIMD (1 024 waves), 8 independent chains per
+// wave-wide shifts: nine per row of the fused Harris kernel), and other kinds beside them.  One wave per SIMD (1 024 waves), 8 independent chains per
 // lane, 4 000 x 8 instructions per wave, 1 .. 4 waves per SIMD (1 024 .. 4 096 one-wave workgroups); prints cycles per instruction from s_memtime.
-//   hipcc --offload-arch=gfx950 -O2 -w -o /tmp/ubench_dpp tools/ubench_dpp.hip && /tmp/ubench_dpp
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -w -o /tmp/ubench_dpp tools/ubench_dpp.hip && /tmp/ubench_dpp
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>
@@ -23,7 +23,6 @@ __global__ __launch_bounds__(64) void k(uint32_t* out, unsigned long long* cyc, 
 #define ROWS(i) asm volatile("v_mov_b32_dpp %0, %0 row_shr:1 row_mask:0xf bank_mask:0xf bound_ctrl:1" : "+v"(r[i]));
 #define WSHR(i) asm volatile("v_mov_b32_dpp %0, %0 wave_shr:1 row_mask:0xf bank_mask:0xf bound_ctrl:1" : "+v"(r[i]));
 #define WSHL(i) asm volatile("v_mov_b32_dpp %0, %0 wave_shl:1 row_mask:0xf bank_mask:0xf bound_ctrl:1" : "+v"(r[i]));
-#define PKAD(i) asm volatile("v_pk_add_f32 %0, %0, %1" : "+v"(*(double*)&f[2 * i]) : "v"(*(double*)&f[(2 * i + 2) & 15]));
 #define PKMV(i) asm volatile("v_pk_mov_b32 %0, %0, %1 op_sel:[1,0]" : "+v"(*(double*)&f[2 * i]) : "v"(*(double*)&f[(2 * i + 2) & 15]));
 #define MAX3(i) asm volatile("v_max3_f32 %0, %0, %1, %2" : "+v"(f[i]) : "v"(f[i + 8]), "v"(f[(i + 1) & 7]));
 #define DOT4(i) asm volatile("v_dot4_u32_u8 %0, %0, %1, %0" : "+v"(r[i]) : "v"(r[(i + 1) & 7]));
@@ -31,19 +30,12 @@ __global__ __launch_bounds__(64) void k(uint32_t* out, unsigned long long* cyc, 
 #define PERM(i) asm volatile("v_perm_b32 %0, %0, %1, %2" : "+v"(r[i]) : "v"(r[(i + 1) & 7]), "s"(0x0c0c0b09u));
 #define SADD(i) asm volatile("s_add_u32 %0, %0, 3" : "+s"(sr[i & 3]));
 #define SNOP(i) asm volatile("s_nop 0");
-#define MIX1(i) asm volatile("v_pk_add_f32 %0, %0, %2\n\ts_add_u32 %1, %1, 3" : "+v"(*(double*)&f[2 * i]), "+s"(sr[i & 3]) : "v"(*(double*)&f[(2 * i + 2) & 15]));
-#define MIX2(i) asm volatile("v_pk_add_f32 %0, %0, %1\n\ts_nop 0" : "+v"(*(double*)&f[2 * i]) : "v"(*(double*)&f[(2 * i + 2) & 15]));
-#define MIX3(i) asm volatile("v_pk_add_f32 %0, %0, %2\n\tv_mov_b32 %1, %1" : "+v"(*(double*)&f[2 * i]), "+v"(r[i]) : "v"(*(double*)&f[(2 * i + 2) & 15]));
         if (KIND == 10) { REP8(SADD) }
         if (KIND == 11) { REP8(SNOP) }
-        if (KIND == 12) { REP8(MIX1) }
-        if (KIND == 13) { REP8(MIX2) }
-        if (KIND == 14) { REP8(MIX3) }
         if (KIND == 0) { REP8(MOVP) }
         if (KIND == 1) { REP8(ROWS) }
         if (KIND == 2) { REP8(WSHR) }
         if (KIND == 3) { REP8(WSHL) }
-        if (KIND == 4) { REP8(PKAD) }
         if (KIND == 5) { REP8(PKMV) }
         if (KIND == 6) { REP8(MAX3) }
         if (KIND == 7) { REP8(DOT4) }
@@ -69,7 +61,7 @@ static void run(const char* name, uint32_t* out, unsigned long long* cyc, int nb
     std::vector<unsigned long long> h(nblocks);
     hipMemcpy(h.data(), cyc, nblocks * sizeof(unsigned long long), hipMemcpyDeviceToHost);
     std::sort(h.begin(), h.end());
-    printf("  %-30s %2d waves per SIMD: a wave issues one every %6.2f cycles = %5.2f cycles of the SIMD per instruction (pairs: per pair)\n", name, nblocks / 1024, (double)h[nblocks / 2] / (iters * 8.0),
+    printf("  %-30s %2d waves per SIMD: a wave issues one every %6.2f cycles = %5.2f cycles of the SIMD per instruction\n", name, nblocks / 1024, (double)h[nblocks / 2] / (iters * 8.0),
            (double)h[nblocks / 2] / (iters * 8.0) / (nblocks / 1024));
 }
 
@@ -84,15 +76,12 @@ int main()
     run<1>("v_mov_b32_dpp row_shr:1", out, cyc, nblocks);
     run<2>("v_mov_b32_dpp wave_shr:1", out, cyc, nblocks);
     run<3>("v_mov_b32_dpp wave_shl:1", out, cyc, nblocks);
-    run<4>("v_pk_add_f32", out, cyc, nblocks);
     run<5>("v_pk_mov_b32 op_sel:[1,0]", out, cyc, nblocks);
     run<6>("v_max3_f32", out, cyc, nblocks);
     run<7>("v_dot4_u32_u8", out, cyc, nblocks);
     run<8>("v_cvt_f32_ubyte2", out, cyc, nblocks);
     run<9>("v_perm_b32", out, cyc, nblocks);
     run<11>("s_nop 0", out, cyc, nblocks);
-    run<13>("pairs: v_pk_add_f32 + s_nop 0", out, cyc, nblocks);
-    run<14>("pairs: v_pk_add_f32 + v_mov_b32", out, cyc, nblocks);
     }
     return 0;
 }
