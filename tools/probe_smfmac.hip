@@ -1,5 +1,5 @@
 // tools/probe_smfmac.hip -- operand layout probe for v_smfmac_i32_16x16x128_i8 on gfx950 (no public layout table at hand).
-//   hipcc -Xclang -target-feature -Xclang -packed-fp32-ops -O2 --offload-arch=gfx950 -o gpurun_out/probe_smfmac tools/probe_smfmac.hip && gpurun_out/probe_smfmac > gpurun_out/smfmac_layout.txt
+//   hipcc -Xclang -target-feature -Xclang -packed-fp32-ops -O2 --offload-arch=gfx950 -o /tmp/probe_smfmac tools/probe_smfmac.hip && /tmp/probe_smfmac > /tmp/smfmac_layout.txt
 // Phase 1: for every stored A element (lane La, byte ja) and 2-bit index code c (all 16 index fields of every lane set to c),
 //   A one-hot, B element (lane Lb, byte jb) carries its own location number 1 + 32*Lb + jb bit by bit over 12 runs:
 //   the D entries that light up give the output row m and, per column n, WHICH B element the A element multiplies.
